@@ -184,6 +184,10 @@ struct DecWarp {
   int tok_per_stage, kv_bytes, stage_bytes, row_bytes, stages;
 };
 
+// What a warp hands on as the maximum of a row: NaN where the row's sum is.  (fmaxf passes NaN by, so a warp whose visible tokens are all NaN
+// has the maximum of one that saw nothing, and the combination would leave it out.)
+__device__ __forceinline__ float max_or_nan(float m, float l) { return l != l ? l : m; }
+
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -445,9 +449,9 @@ __device__ __forceinline__ void consume_plain(const DecodeArgs& a, const DecWarp
         w.mine[rr * kCmbRow + j * 8 + 2 * c + (e & 1)] = acc[mt][j][e];
       }
     if (c == 0) {
-      w.mine[(mt * 16 + r) * kCmbRow + D] = m_run[mt][0];
+      w.mine[(mt * 16 + r) * kCmbRow + D] = max_or_nan(m_run[mt][0], l_run[mt][0]);
       w.mine[(mt * 16 + r) * kCmbRow + D + 1] = l_run[mt][0];
-      w.mine[(mt * 16 + r + 8) * kCmbRow + D] = m_run[mt][1];
+      w.mine[(mt * 16 + r + 8) * kCmbRow + D] = max_or_nan(m_run[mt][1], l_run[mt][1]);
       w.mine[(mt * 16 + r + 8) * kCmbRow + D + 1] = l_run[mt][1];
     }
   }
@@ -684,7 +688,7 @@ __device__ __forceinline__ void quant_rows_finish(QuantRows<NTQ>& q, const DecWa
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float* row = w.mine + (nt * 8 + 2 * c + e) * cmb_pitch(D);
-        row[D] = q.slack[nt][e] == -INFINITY ? -INFINITY : q.ref[nt][e];
+        row[D] = max_or_nan(q.slack[nt][e] == -INFINITY ? -INFINITY : q.ref[nt][e], q.l[nt][e]);
         row[D + 1] = q.l[nt][e];
       }
   }
@@ -1222,7 +1226,7 @@ __device__ __forceinline__ void consume_int4_groups(const DecodeArgs& a, const D
     if (r == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        w.mine[(nt * 8 + 2 * c + e) * kCmbRow + D] = m_run[nt][e];
+        w.mine[(nt * 8 + 2 * c + e) * kCmbRow + D] = max_or_nan(m_run[nt][e], l_run[nt][e]);
         w.mine[(nt * 8 + 2 * c + e) * kCmbRow + D + 1] = l_run[nt][e];
       }
     }
@@ -1735,8 +1739,8 @@ __global__ void __launch_bounds__(kDecThreads, DecOccupancy<kFmt, MT>::kCtasPerS
       else
         combine(std::integral_constant<int, kDecConsumerWarps>{});
     }
-    const float inv = den > 0.f ? 1.f / den : 0.f;
-    const float lse = den > 0.f ? (m_use + log2f(den)) * 0.6931471805599453f : -INFINITY;
+    const float inv = den != 0.f ? 1.f / den : 0.f;  // (a sum of NaN stays one)
+    const float lse = den != 0.f ? (m_use + log2f(den)) * 0.6931471805599453f : -INFINITY;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     const int row = row0 + rr, oh = hblk * hb + hh;
     if (direct) {
@@ -1816,21 +1820,21 @@ __global__ void __launch_bounds__(kMergeWarpsPerCta * 32) decode_merge_kernel(co
   };
   load(part);
   float mx = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) mx = fmaxf(mx, a.part_lse[prow0 + s * pstep]);
+  for (int s = lane; s < nsplit; s += 32) mx = fmax_nan(mx, a.part_lse[prow0 + s * pstep]);  // (NaN in any chunk is NaN in all that follows)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  for (int o = 16; o > 0; o >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
   float den = 0.f;
-  if (mx > -INFINITY) {
+  if (mx != -INFINITY) {
     for (int s0 = part;;) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float w = l[u] > -INFINITY ? __expf(l[u] - mx) : 0.f;
+        const float w = l[u] != -INFINITY ? __expf(l[u] - mx) : 0.f;
         den += w;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += l[u] > -INFINITY ? w * x[u][i] : 0.f;  // (0 x NaN stays NaN)
+        for (int i = 0; i < V; ++i) acc[i] += l[u] != -INFINITY ? w * x[u][i] : 0.f;  // (0 x NaN stays NaN)
       }
       s0 += U * step;
       if (s0 >= nsplit) break;
@@ -1848,7 +1852,7 @@ __global__ void __launch_bounds__(kMergeWarpsPerCta * 32) decode_merge_kernel(co
     for (int i = 0; i < V; ++i) acc[i] += red[warp + w][lane * V + i];
     den += red[warp + w][D];
   }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = den != 0.f ? 1.f / den : 0.f;
   const int qi = row / a.q_per_kv, h = row % a.q_per_kv;
   const int64_t off = (int64_t(b) * a.mq + qi) * a.o_sm + int64_t(head) * a.o_sg + int64_t(h) * a.o_sh + lane * V;
 #pragma unroll
@@ -1862,7 +1866,7 @@ __global__ void __launch_bounds__(kMergeWarpsPerCta * 32) decode_merge_kernel(co
       reinterpret_cast<__half*>(a.out)[off + i] = __float2half_rn(val);
   }
   if (a.lse != nullptr && lane == 0)
-    a.lse[int64_t(head) * a.lse_sg + int64_t(h) * a.lse_sh + int64_t(b) * a.mq + qi] = den > 0.f ? mx + __logf(den) : -INFINITY;
+    a.lse[int64_t(head) * a.lse_sg + int64_t(h) * a.lse_sh + int64_t(b) * a.mq + qi] = den != 0.f ? mx + __logf(den) : -INFINITY;
 }
 
 // ------------------------------------------------------------------ host side

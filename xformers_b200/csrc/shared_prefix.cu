@@ -852,7 +852,7 @@ struct MergeLoads {
   __device__ __forceinline__ void add(float mx, float (&acc)[V], float& den) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // (NaN goes on; the decode kernel gives a row that saw NaN the log-sum-exp of one that saw nothing, but the columns of that one are zero)
+      // (NaN goes on; the prefill kernels give a row that saw NaN the log-sum-exp of one that saw nothing, but the columns of that one are zero)
       const float w = l[u] != -INFINITY ? __expf(l[u] - mx) : 0.f * x[u][0];
       den += w;
 #pragma unroll
