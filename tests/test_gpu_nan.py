@@ -18,9 +18,6 @@ NAN_WORD = 0x7E007E00  # scale and shift of a quantised row: fp16 NaN
 LENS, BAD = [1, 17, 129, 700, 700, 40, 0], [0, 16, 128, 699, 3, None, None]
 
 
-def _same(a, b):
-    return torch.equal(a.nan_to_num(nan=123.0), b.nan_to_num(nan=123.0))
-
 
 def _check(out, lse, clean, clean_lse, bad):
     """out [tokens, ..], lse [.., tokens], `bad` [tokens]: rows that see NaN."""
@@ -121,3 +118,55 @@ def test_own_keys_behind_a_shared_prefix(prefix, lens, bad, pad, page):
             c.own.k[0, c.own.where[i][t]] = float("nan")
     out, lse = c.call(return_lse=True)
     _check(out[0], lse[0], clean[0], clean_lse[0], torch.tensor([t is not None for t in bad], device="cuda"))
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 300])
+@pytest.mark.parametrize("q_len,kv_len", [([7, 1, 40, 12, 9], [7, 300, 60, 12, 30]), ([150, 1, 200, 70, 9], [150, 5, 260, 200, 9])])
+@pytest.mark.parametrize("through_front", [True, False])
+def test_prefill_of_own_keys_behind_a_shared_prefix(prefix, q_len, kv_len, through_front, monkeypatch):
+    """Unequal token counts: the partials are a prefill kernel's.  NaN in the only key that a token sees, among others, in the newest key, in a hidden value."""
+    from xformers_b200 import _lib
+
+    if not through_front:
+        monkeypatch.setattr(_lib, "front", None)
+    c = Case([sum(q_len)], [prefix], q_len, kv_len, seed=prefix + len(q_len))
+    clean, clean_lse = c.call(return_lse=True)
+    c.check((clean, clean_lse))
+    at = [0, kv_len[1] - 1, kv_len[2] // 2, kv_len[3] - 1, None]
+    bad = []
+    for i, (n, m, t) in enumerate(zip(q_len, kv_len, at)):
+        bad += [t is not None and m - n + j >= t for j in range(n)]
+        if t is not None:
+            c.own.k[0, c.own.where[i][t]] = float("nan")
+    out, lse = c.call(return_lse=True)
+    _check(out[0], lse[0], clean[0], clean_lse[0], torch.tensor(bad, device="cuda"))
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+def test_tokens_without_own_keys_on_the_prefill_path(prefix):
+    """A sequence without own keys, and tokens ahead of the first own key of theirs, whose tile holds NaN that only later tokens see."""
+    c = Case([60], [prefix], [9, 11, 40], [9, 0, 25], seed=31)
+    clean, clean_lse = c.call(return_lse=True)
+    c.check((clean, clean_lse))
+    if prefix == 0:
+        assert bool((clean[0, 9:35] == 0).all()) and bool((clean_lse[..., 9:35] == float("-inf")).all())
+    c.own.k[0, c.own.where[2][24]] = c.own.v[0, c.own.where[2][24]] = float("nan")  # of the last token alone
+    out, lse = c.call(return_lse=True)
+    assert torch.equal(out[:, :35], clean[:, :35]) and torch.equal(lse[..., :59], clean_lse[..., :59])
+    assert bool(out[:, 59].isnan().all()) and bool(lse[..., 59].isnan().all())
+
+
+@pytest.mark.parametrize("op", ["FwOp_Tcgen05_Persistent", "FwOp_Tcgen05_M256", "FwOp_Generic"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill(op, d):
+    """The log-sum-exp of a row that sees NaN is NaN, in each of the prefill kernels."""
+    gen = torch.Generator().manual_seed(d)
+    q_len, kv_len = [300, 5, 130], [300, 70, 133]
+    q = torch.randn(1, sum(q_len), 4, d, generator=gen).bfloat16().cuda()
+    k, v = (torch.randn(1, sum(kv_len), 4, d, generator=gen).bfloat16().cuda() for _ in range(2))
+    bias = ab.BlockDiagonalCausalFromBottomRightMask.from_seqlens(q_len, kv_len, device="cuda")
+    run = lambda: [x[0] for x in fmha.memory_efficient_attention_forward_requires_grad(q, k, v, bias, op=getattr(fmha.b200, op))]
+    clean = run()
+    k[0, 0], k[0, 300 + 69], k[0, 370 + 100] = (float("nan"),) * 3
+    bad = [True] * 300 + [False] * 4 + [True] + [3 + j >= 100 for j in range(130)]
+    _check(*run(), *clean, torch.tensor(bad, device="cuda"))

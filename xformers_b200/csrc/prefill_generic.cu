@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kGenThreads) prefill_generic_kernel(const __gr
   for (int hlf = 0; hlf < 2; ++hlf) {
     const int i = hlf ? i1 : i0;
     if (i >= qlen) continue;
-    const float inv = l_run[hlf] > 0.f ? 1.f / l_run[hlf] : 0.f;
+    const float inv = l_run[hlf] != 0.f ? 1.f / l_run[hlf] : 0.f;
     const int64_t off = qb * p.o_strides.b + (q_row0 + i) * p.o_strides.m + int64_t(g) * p.o_strides.g + int64_t(h) * p.o_strides.h;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kGenThreads) prefill_generic_kernel(const __gr
       }
     }
     if (p.lse != nullptr && c == 0) {
-      const float lse = l_run[hlf] > 0.f ? (m_run[hlf] + log2f(l_run[hlf])) * 0.6931471805599453f : -INFINITY;
+      const float lse = l_run[hlf] != 0.f ? (m_run[hlf] + log2f(l_run[hlf])) * 0.6931471805599453f : -INFINITY;
       const int64_t lo = p.seqstart_q != nullptr ? int64_t(g) * p.lse_stride_g + int64_t(h) * p.lse_stride_h + q_row0 + i
                                                  : int64_t(b) * p.lse_stride_b + int64_t(g) * p.lse_stride_g + int64_t(h) * p.lse_stride_h + i;
       p.lse[lo] = lse;

@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_sm100_m256_kernel(const _
       tc_fence_after();
     }
     const bool valid_row = i_loc < qlen;
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
     const int64_t o_off = int64_t(tb) * a.os.b + int64_t(q_row0 + i_loc) * a.os.m + int64_t(g) * a.os.g + int64_t(h) * a.os.h;
 #pragma unroll
     for (int cblk = 0; cblk < D / 32; ++cblk) {
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_sm100_m256_kernel(const _
       }
     }
     if (valid_row && a.lse != nullptr) {
-      const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+      const float lse = l_run != 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
       const int64_t lo = a.seqstart_q != nullptr ? int64_t(g) * a.lse_g + int64_t(h) * a.lse_h + q_row0 + i_loc
                                                  : int64_t(b) * a.lse_b + int64_t(g) * a.lse_g + int64_t(h) * a.lse_h + i_loc;
       a.lse[lo] = lse;

@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_sm100_persist_kernel(cons
             oph ^= 1u << t;
             tc_fence_after();
           }
-          const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+          const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
           const int64_t o_off = int64_t(it.tb) * a.os.b + int64_t(it.q_row0 + i_loc) * a.os.m + int64_t(it.g) * a.os.g + int64_t(it.h + h_loc) * a.os.h;
 #pragma unroll 1
           for (int col = 0; col < D; col += 16) {
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_sm100_persist_kernel(cons
             }
           }
           if (valid_row && a.lse != nullptr) {
-            const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+            const float lse = l_run != 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
             const int64_t lo = a.seqstart_q != nullptr ? int64_t(it.g) * a.lse_g + int64_t(it.h + h_loc) * a.lse_h + it.q_row0 + i_loc
                                                        : int64_t(it.b) * a.lse_b + int64_t(it.g) * a.lse_g + int64_t(it.h + h_loc) * a.lse_h + i_loc;
             a.lse[lo] = lse;

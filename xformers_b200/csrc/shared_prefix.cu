@@ -852,26 +852,20 @@ struct MergeLoads {
   __device__ __forceinline__ void add(float mx, float (&acc)[V], float& den) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // (NaN goes on; the prefill kernels give a row that saw NaN the log-sum-exp of one that saw nothing, but the columns of that one are zero)
-      const float w = l[u] != -INFINITY ? __expf(l[u] - mx) : 0.f * x[u][0];
+      const float w = l[u] != -INFINITY ? __expf(l[u] - mx) : 0.f;
       den += w;
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += w * x[u][i];
+      for (int i = 0; i < V; ++i) acc[i] += l[u] != -INFINITY ? w * x[u][i] : 0.f;  // (NaN goes on; a partial without a visible key counts for nothing, whatever its columns hold)
     }
   }
 };
-// Largest log-sum-exp of a row, by a warp; false: no partial with a visible key (or with NaN among them).
-__device__ __forceinline__ bool merge_max(const MergeArgs& a, const MergeRow& row, int lane, float& mx) {
-  bool any = false;
-  mx = -INFINITY;
-  for (int s = lane; s < row.n; s += 32) {
-    const float e = merge_lse(a, row, s);
-    any |= e != -INFINITY;
-    mx = fmaxf(mx, e);
-  }
+// Largest log-sum-exp of a row, by a warp: -inf if no partial has a visible key, NaN if one of them saw NaN.
+__device__ __forceinline__ float merge_max(const MergeArgs& a, const MergeRow& row, int lane) {
+  float mx = -INFINITY;
+  for (int s = lane; s < row.n; s += 32) mx = fmax_nan(mx, merge_lse(a, row, s));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  return __any_sync(0xffffffffu, any);
+  for (int o = 16; o > 0; o >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  return mx;
 }
 template <int V>
 __device__ __forceinline__ void merge_store(const MergeArgs& a, const MergeRow& row, int lane, float mx, const float (&acc)[V], float den) {
@@ -931,14 +925,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const __
   float mx = -INFINITY, acc[V], den = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  bool any = false;
   if (step == 1 && row.n <= U) {  // (all of them are here)
 #pragma unroll
-    for (int u = 0; u < U; ++u) any |= now.l[u] != -INFINITY, mx = fmaxf(mx, now.l[u]);
+    for (int u = 0; u < U; ++u) mx = fmax_nan(mx, now.l[u]);
   } else {
-    any = merge_max(a, row, lane, mx);
+    mx = merge_max(a, row, lane);
   }
-  if (any) {
+  if (mx != -INFINITY) {
     for (int s0 = part;;) {
       now.add(mx, acc, den);
       s0 += U * step;
