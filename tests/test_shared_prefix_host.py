@@ -138,3 +138,36 @@ def test_scratch():
     p.own = C.pointer(own)
     part = 5 * 3 * 2 * 4
     assert lib.xfb200_shared_prefix_scratch_bytes(C.byref(p)) == up(32) + up(slots * rows * 64 * 4) + up(slots * rows * 4) + up(part * 64 * 4) + up(part * 4)
+
+
+@pytest.mark.parametrize("words", [0, 17, 32])
+@pytest.mark.parametrize("batch,pad,layout", [(4, 4096, (8, 4)), (8, 8192, (8, 8)), (1, 700, (1, 16)), (128, 2056, (8, 8)), (40, 300, (4, 7))])
+def test_both_paths_cut_the_own_keys_alike(words, batch, pad, layout):
+    """The chunks that the Python path asks for are those of the C rule, whose arguments the host front passes in C order."""
+    from xformers_b200.ops.fmha import b200_splitk, common, shared_prefix
+
+    G, H = layout
+    q = torch.zeros(1, batch, G, H, 128, dtype=torch.bfloat16)
+    key = torch.zeros(1, 1, G, 1, words or 128, dtype=torch.int32 if words else q.dtype).expand(-1, batch * pad, -1, H, -1)
+    bias = ab.BlockDiagonalCausalWithOffsetPaddedKeysMask.from_seqlens(q_seqlen=[1] * batch, kv_padding=pad, kv_seqlen=[pad] * batch)
+    extra = {f"{n}_fp8_scale_shift": torch.zeros(1, 1, G, H, dtype=torch.int32).expand(-1, batch * pad, -1, -1) for n in "kv"} if words == 32 else {}
+    inp = (common.InputsFp8 if extra else common.Inputs)(q, key, key, bias, 0.0, None, torch.float32, True, **extra)
+    q5, k5, v5, broadcast = b200_splitk._geometry(inp)
+    p = b200_splitk.FwOp.params(inp, k5, v5, q5, broadcast, shared_prefix._split_k)
+    rows, row_bytes = H, (words or 64) * 4
+    assert p.split_k == _lib.load().xfb200_shared_prefix_split_k(batch, pad, G, rows, row_bytes, int(words > 0))
+    assert b200_splitk.FwOp.params(inp, k5, v5, q5, broadcast).split_k == _lib.load().xfb200_decode_split_k(batch, pad, G, rows, row_bytes, int(words > 0))
+
+
+def test_the_rule_gets_its_arguments_in_c_order(monkeypatch):
+    from xformers_b200.ops.fmha import shared_prefix
+
+    seen, lib = {}, _lib.load()
+
+    def rule(batch, kv_bound, kv_heads, rows, row_bytes, quantised):
+        seen.update(rows=rows, row_bytes=row_bytes, kv_heads=kv_heads)
+        return 1
+
+    monkeypatch.setattr(lib, "xfb200_shared_prefix_split_k", rule)
+    assert shared_prefix._split_k(3, 100, 2, 256, 12, False) == 1
+    assert seen == dict(rows=12, row_bytes=256, kv_heads=2)

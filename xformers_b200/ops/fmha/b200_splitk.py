@@ -238,7 +238,7 @@ class FwOp(AttentionFwOpBase):
 
     @classmethod
     def params(cls, inp: Inputs, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor, broadcast: bool, split_k=None) -> _lib.DecodeParams:
-        """The C parameters of a call, all but the outputs and the scratch (``split_k``: the rule for the split count, ``get_split_k``)."""
+        """The C parameters of a call, all but the outputs and the scratch (``split_k``: the rule for the split count in place of ``get_split_k``, with its arguments in the same order)."""
         B, Mq, G, H, D = q.shape
         bias = inp.attn_bias
         quantized = k.dtype == torch.int32

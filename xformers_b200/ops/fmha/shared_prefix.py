@@ -84,6 +84,11 @@ def _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, 
             raise NotImplementedError(f"{name}: rows of {what} must be contiguous and start on 16-byte boundaries")
 
 
+def _split_k(batch: int, kv_bound: int, kv_heads: int, row_bytes: int, rows: int, quantised: bool) -> int:
+    """``xfb200_shared_prefix_split_k`` with its arguments in the order of ``FwOp.get_split_k``."""
+    return _lib.load().xfb200_shared_prefix_split_k(batch, kv_bound, kv_heads, rows, row_bytes, quantised)
+
+
 def _debug_check(prefix_bias, rows: int) -> None:
     lens, bound = prefix_bias.k_seqinfo.seqlen.cpu().tolist(), prefix_bias.k_seqinfo.padding
     if isinstance(prefix_bias, ab.PagedBlockDiagonalPaddedKeysMask):
@@ -192,7 +197,7 @@ def shared_prefix_attention(
                 _debug_check(prefix_bias, p.kv_rows)
             own = None
             if type(attn_bias) in _DECODE_BIASES and not b200_splitk.FwOp.not_supported_reasons(inp):
-                own = b200_splitk.FwOp.params(inp, ok, ov, q, own_broadcast, lib.xfb200_shared_prefix_split_k if b200_splitk.FwOp.SPLIT_K is None else None)
+                own = b200_splitk.FwOp.params(inp, ok, ov, q, own_broadcast, _split_k if b200_splitk.FwOp.SPLIT_K is None else None)
                 p.own = C.pointer(own)
             else:
                 from . import _run_forward
