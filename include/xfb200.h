@@ -144,7 +144,9 @@ typedef struct {
    * leaves that many SMs free, for kernels of other streams that are meant to run beside it (the
    * collectives that exchange one stripe of a sharded sequence while the next one is computed). */
   int32_t sm_margin;
-  int32_t reserved;
+  /* 1: the kernel does not begin before everything ahead of it in the stream has ended, not even with what it does before it touches memory.  For a
+   * call that another one is to run beside (own_beside of xfb200_shared_prefix_params) */
+  int32_t in_order;
 } xfb200_prefill_params;
 
 XFB200_API int xfb200_prefill_forward(const xfb200_prefill_params* p, void* stream);
@@ -224,8 +226,8 @@ typedef struct {
   /* 0, or a sum of
    * XFB200_DECODE_PARTIALS_ONLY: the partials of the chunks are left in scratch, with a single chunk as well, and not merged
    *   (xfb200_shared_prefix_forward joins them with those of a prefix); out and lse are not written;
-   * XFB200_DECODE_BESIDE: the launch may run beside the one ahead of it in the stream, which must be a kernel of this library that has waited
-   *   for whatever wrote this call's inputs before it lets the next one begin, and that does not touch what this call writes;
+   * XFB200_DECODE_BESIDE: the launch may run beside the one ahead of it in the stream, which must be a kernel of this library that did not begin
+   *   before everything ahead of it had ended (an ordinary launch), that did not write this call's inputs and that does not touch what this call writes;
    * XFB200_DECODE_ONE_TILE: a CTA has one tile of query rows, whatever their number (for sequences of few keys, which more CTAs read sooner). */
   int32_t flags;
   /* Additive bias (a plain tensor as attn_bias; the reference's split-K operator takes one,
@@ -313,8 +315,8 @@ typedef struct {
   int32_t kv_heads, q_per_kv, head_dim;
   int32_t kv_padding; /* most keys of a prefix; padded: the slot size; 0: there are none */
   int32_t page_size;
-  /* 1: the kernel ahead in the stream is the one that leaves own_out / own_lse, one of this library's that has waited for whatever wrote this call's
-   * other inputs before it lets the next one begin, and that does not touch out, lse or scratch: the prefixes may be read beside it */
+  /* 1: the kernel ahead in the stream is the one that leaves own_out / own_lse, one of this library's that did not begin before everything ahead of it had
+   * ended (in_order of xfb200_prefill_params), and that does not touch out, lse or scratch: the prefixes may be read beside it */
   int32_t own_beside;
   float scale; /* positive */
   int64_t block_table_stride;

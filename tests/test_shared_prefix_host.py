@@ -171,3 +171,15 @@ def test_the_rule_gets_its_arguments_in_c_order(monkeypatch):
     monkeypatch.setattr(lib, "xfb200_shared_prefix_split_k", rule)
     assert shared_prefix._split_k(3, 100, 2, 256, 12, False) == 1
     assert seen == dict(rows=12, row_bytes=256, kv_heads=2)
+
+
+def test_prefill_refuses_another_launch_order():
+    lib = _lib.load()
+    p = _lib.PrefillParams()
+    p.batch = p.mq = p.mkv = p.total_q = p.groups = p.heads_per_group = 1
+    p.head_dim, p.dtype, p.out_dtype, p.window_left = 64, _lib.BF16, _lib.BF16, -1
+    p.q = p.k = p.v = p.out = 256
+    for value in (-1, 2):
+        p.in_order = value
+        assert lib.xfb200_prefill_forward(C.byref(p), None) == _lib.XFB200_E_INVALID
+        assert b"in_order" in lib.xfb200_last_error()

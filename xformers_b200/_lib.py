@@ -94,7 +94,7 @@ class PrefillParams(C.Structure):
         ("kv_split", C.c_int32),
         ("kv_offset2", C.c_int32),
         ("sm_margin", C.c_int32),
-        ("reserved", C.c_int32),
+        ("in_order", C.c_int32),
     ]
 
 

@@ -1429,11 +1429,11 @@ __global__ void __launch_bounds__(kDecThreads, DecOccupancy<kFmt, MT>::kCtasPerS
     if (a.copy_mode == 3) prefetch_tensormap(&a.tm_k), prefetch_tensormap(&a.tm_v);
   }
   // (In this order: the merge reads the lengths before its own wait, so it must not begin before whatever wrote them has ended.)
-  // Beside the kernel ahead (XFB200_DECODE_BESIDE): that one has waited for everything this one reads.  The launch's last CTA waits for it at
+  // Beside the kernel ahead (XFB200_DECODE_BESIDE): everything this one reads was complete when that one began.  The launch's last CTA waits for it at
   // its end, so that whoever waits for this kernel has both; the others would only keep their SMs.
   const bool wait_at_end = a.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
   if (a.beside)
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");  // (what an earlier kernel left in this SM's L1 may be out of date)
+    beside_fence();
   else
     grid_dep_wait();
   grid_dep_launch();

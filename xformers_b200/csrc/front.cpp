@@ -137,8 +137,8 @@ py::object result(const Tensor& out, const OptTensor& lse) { return py::make_tup
 
 Tensor new_out(const View& q, at::ScalarType dt) { return at::empty(q.t.sizes(), q.t.options().dtype(dt)); }
 
-// Runs a prefill; false: not one that the kernels cover.
-bool run_prefill(const View& q, const View& k, const View& v, const Sequences* s, const Call& c, Tensor& out, OptTensor& lse) {
+// Runs a prefill (in_order: an ordinary launch); false: not one that the kernels cover.
+bool run_prefill(const View& q, const View& k, const View& v, const Sequences* s, const Call& c, Tensor& out, OptTensor& lse, bool in_order = false) {
   const int64_t D = q.D;
   if (!(c.flags & kPrefillTakesBias)) return false;
   const int dt = dtype_code(q.t.scalar_type()), odt = dtype_code(c.out_dtype);
@@ -160,7 +160,7 @@ bool run_prefill(const View& q, const View& k, const View& v, const Sequences* s
   out = new_out(q, c.out_dtype);
   const auto f32 = q.t.options().dtype(at::kFloat);
   if (lse_wanted) lse = q.five ? at::empty({q.B, q.G, q.H, q.M}, f32) : at::empty({q.B, q.H, q.M}, f32);
-  p.q = q.t.data_ptr(), p.k = k.t.data_ptr(), p.v = v.t.data_ptr(), p.out = out.data_ptr();
+  p.q = q.t.data_ptr(), p.k = k.t.data_ptr(), p.v = v.t.data_ptr(), p.out = out.data_ptr(), p.in_order = in_order;
   p.lse = lse_wanted ? lse->data_ptr<float>() : nullptr;
   p.dtype = dt, p.out_dtype = odt;
   if (s != nullptr) {
@@ -421,8 +421,8 @@ py::object shared(const Tensor& q_, const Tensor& pk_, const Tensor& pv_, const 
     if (!decode_params(q, k, v, &s, c, own, g_shared_split_k)) return py::none();
     p.own = &own;
   } else {
-    if (max_q < 1 || s.tables != nullptr || k_.scalar_type() == at::kInt || !run_prefill(q, k, v, &s, c, own_out, own_lse)) return py::none();
-    p.own_out = own_out.data_ptr<float>(), p.own_lse = own_lse->data_ptr<float>(), p.own_beside = 1;  // (run_prefill has launched one kernel, which has no other outputs)
+    if (max_q < 1 || s.tables != nullptr || k_.scalar_type() == at::kInt || !run_prefill(q, k, v, &s, c, own_out, own_lse, true)) return py::none();
+    p.own_out = own_out.data_ptr<float>(), p.own_lse = own_lse->data_ptr<float>(), p.own_beside = 1;  // (run_prefill has launched one kernel, in order, which has no other outputs)
     p.own_stride_m = q.G * q.H * D, p.own_stride_g = broadcast ? osg : D, p.own_stride_h = broadcast ? D : 0;
     p.own_lse_stride_g = broadcast ? q.H * q.M : q.M, p.own_lse_stride_h = broadcast ? q.M : 0;
   }

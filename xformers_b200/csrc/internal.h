@@ -89,17 +89,23 @@ inline size_t decode_partials_bytes(const xfb200_decode_params& p) {
 // of a decoding step's 3-6 us kernels.  In a captured stream it becomes an edge of the same kind.
 //   A kernel that leaves SMs free for other streams (sm_margin) neither is launched this way nor lets the next one begin: CTAs that
 // only wait would fill those SMs.
+//   in_order: an ordinary launch, for the first of two kernels that run beside one another.  What griddepcontrol.wait makes visible, it makes visible to the grid that waits; a
+// kernel that runs beside the one ahead of it does not wait, so what both read must have been complete when the first one began.
 template <typename... P>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P&... args) {
+cudaError_t launch_ordered(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool in_order, const P&... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cfg.attrs = &attr, cfg.numAttrs = in_order ? 0 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) cudaGetLastError();  // (returned, not kept)
   return e;
+}
+template <typename... P>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P&... args) {
+  return launch_ordered(kernel, grid, block, smem, stream, false, args...);
 }
 
 }  // namespace xfb

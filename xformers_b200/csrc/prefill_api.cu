@@ -37,6 +37,7 @@ extern "C" int xfb200_prefill_forward(const xfb200_prefill_params* p, void* stre
   if (((p->o_strides.b | p->o_strides.m | p->o_strides.g | p->o_strides.h) * osz) % 8 || (reinterpret_cast<uintptr_t>(p->out) & 7))
     return set_error(XFB200_E_INVALID, "prefill: out rows must be 8-byte aligned");
 
+  if (p->in_order < 0 || p->in_order > 1) return set_error(XFB200_E_INVALID, "prefill: in_order %d", p->in_order);
   if (p->kv_split != 0) {
     if (p->kv_split < 0 || p->kv_split >= p->mkv || p->kv_split % 128 != 0)
       return set_error(XFB200_E_INVALID, "prefill: kv_split %d must be a multiple of 128 inside (0, mkv)", p->kv_split);

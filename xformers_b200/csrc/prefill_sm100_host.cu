@@ -111,6 +111,7 @@ int prefill_sm100_launch(const xfb200_prefill_params* p, cudaStream_t stream) {
   a.window_right = p->mask_type == XFB200_MASK_NONE ? -1 : p->mask_type == XFB200_MASK_LOCAL_BOTTOM_RIGHT ? p->window_right : 0;
   a.kv_split = p->kv_split, a.kv_offset2 = p->kv_offset2;
   a.sm_margin = p->sm_margin > 0 ? p->sm_margin : 0;
+  a.in_order = p->in_order != 0;
   {
     // Work items are handed out heaviest first inside groups of (batch, head) pairs whose keys and values fit the L2
     // together (measured on 4 x 4096 x 32 heads: 945 -> 1020 TFLOP/s causal with 16 or 32 heads per group against all

@@ -1208,7 +1208,7 @@ static int launch_t(Sm100Args a, cudaStream_t stream) {
     kern<<<grid, kThreads, smem, stream>>>(a);
     return check_launch("prefill_sm100_persist_kernel");
   }
-  const cudaError_t e = launch_early(kern, grid, kThreads, smem, stream, a);
+  const cudaError_t e = launch_ordered(kern, grid, kThreads, smem, stream, a.in_order != 0, a);
   return e != cudaSuccess ? cuda_fail("prefill_sm100_persist_kernel launch", e) : XFB200_OK;
 }
 

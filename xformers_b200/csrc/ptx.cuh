@@ -303,6 +303,13 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// In front of what a kernel reads that runs beside the one ahead of it in the stream, which began when all of that was complete: nothing older may be taken from this SM's
+// L1, nor by the copies of the asynchronous proxy.
+__device__ __forceinline__ void beside_fence() {
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
 // Pairs of fp32 values in 64-bit registers, two operations an instruction.
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
   uint64_t r;

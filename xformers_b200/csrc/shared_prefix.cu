@@ -244,10 +244,10 @@ __global__ void __launch_bounds__(threads(kTiles), 1) shared_prefix_kernel(const
     if (a.q_tma) prefetch_tensormap(&a.tm_q);
   }
   __syncwarp();
-  // Beside the kernel ahead (xfb200_shared_prefix_params.own_beside): that one has waited for everything this one reads.  The last CTA waits for it at its end, so
-  // that whoever waits for this kernel has both.
+  // Beside the kernel ahead (xfb200_shared_prefix_params.own_beside): everything this one reads was complete when that one began.  The last CTA waits for it at its
+  // end, so that whoever waits for this kernel has both.
   if (a.beside)
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");  // (what an earlier kernel left in this SM's L1 may be out of date)
+    beside_fence();
   else
     grid_dep_wait();
   grid_dep_launch();
@@ -899,7 +899,7 @@ __device__ __forceinline__ void merge_store(const MergeArgs& a, const MergeRow& 
   if (a.lse != nullptr && lane == 0) a.lse[int64_t(row.head) * a.lse_sg + int64_t(row.h) * a.lse_sh + row.tok] = den == 0.f ? -INFINITY : mx + __logf(den);
 }
 
-// Before the wait for the kernel ahead: what neither kernel ahead writes.  (Whatever wrote it has ended: each of them lets the next one begin behind its own wait.)
+// Before the wait for the kernel ahead: what neither kernel ahead writes, where there is a prefix kernel: whatever wrote it had ended when the first of the call's kernels began (launch_prefix).
 template <int D, int kWarpsPerRow, int U>
 __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const __grid_constant__ MergeArgs a) {
   constexpr int V = D / 32, step = kWarpsPerRow;
@@ -910,6 +910,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const __
   const uint32_t gh = gw / uint32_t(a.q_per_kv);
   MergeRow row;
   row.h = int(gw - gh * a.q_per_kv), row.tok = live ? int(gh / uint32_t(a.kv_heads)) : 0, row.head = int(gh % uint32_t(a.kv_heads));
+  if (!a.has_prefix) grid_dep_wait();
   const int g = merge_group_of(a, row.tok), q0 = a.has_prefix ? __ldcg(a.seqstart_q + g) : 0;
   merge_own(a, row);
   GroupPlan gp{};
@@ -959,6 +960,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const __
 // ------------------------------------------------------------------ host side
 template <int D, bool kBf16, int kTiles>
 static int launch_prefix(const Args& a, dim3 grid, cudaStream_t st) {
+  // In order, so that the kernels behind it may read beside it what it reads (the decode kernel and the lengths of the merge), or beside a kernel that was launched so.
   auto kern = shared_prefix_kernel<D, kBf16, kTiles>;
   constexpr int smem = Smem<D, kTiles>::kTotal;
   static bool configured[kMaxDevices] = {false};  // the attribute belongs to the device's context
@@ -966,7 +968,7 @@ static int launch_prefix(const Args& a, dim3 grid, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail("shared_prefix: cudaFuncSetAttribute", e);
   }
-  const cudaError_t e = launch_early(kern, grid, threads(kTiles), smem, st, a);
+  const cudaError_t e = launch_ordered(kern, grid, threads(kTiles), smem, st, !a.beside, a);
   return e != cudaSuccess ? cuda_fail("shared_prefix_kernel launch", e) : XFB200_OK;
 }
 
