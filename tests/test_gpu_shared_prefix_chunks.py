@@ -50,3 +50,12 @@ def test_front_and_python_path_agree_over_chunks(fmt, own_page, new, own_pad, la
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     # (a quantised cache: V times its scale is rounded to f16 as well, a half step more)
     c.check(a, c.reference(own=held), slack=1.0 if fmt == "16 bits" else 2.0)
+
+
+@pytest.mark.parametrize("q_len", [[1, 1, 1], [40, 3, 70]])
+@pytest.mark.parametrize("both", [True, False])
+def test_scale_words_beside_16_bit_keys_are_refused(q_len, both):
+    c = Case([sum(q_len)], [300], q_len, [90, 30, 70], seed=3)
+    words = torch.zeros(1, c.own.k.shape[1], 2, 4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="go together"):
+        c.call(k_fp8_scale_shift=words, v_fp8_scale_shift=words if both else None)

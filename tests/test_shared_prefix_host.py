@@ -173,6 +173,19 @@ def test_the_rule_gets_its_arguments_in_c_order(monkeypatch):
     assert seen == dict(rows=12, row_bytes=256, kv_heads=2)
 
 
+_WORDS = torch.zeros(1, 40, 2, 3, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("k_words,v_words,as_words", [(_WORDS, None, True), (None, _WORDS, True), (_WORDS, _WORDS, False), (_WORDS, None, False)])
+def test_scale_words_without_what_they_scale_are_refused(k_words, v_words, as_words):
+    """Not left out of account: words for one of both, or beside 16-bit keys."""
+    a = _args()
+    if as_words:
+        a["key"] = a["value"] = torch.zeros(1, 40, 2, 1, 16, dtype=torch.int32).expand(-1, -1, -1, 3, -1)
+    with pytest.raises(ValueError, match="k_fp8_scale_shift and v_fp8_scale_shift go together"):
+        shared_prefix_attention(**a, k_fp8_scale_shift=k_words, v_fp8_scale_shift=v_words)
+
+
 def test_prefill_refuses_another_launch_order():
     lib = _lib.load()
     p = _lib.PrefillParams()

@@ -356,6 +356,7 @@ py::object shared(const Tensor& q_, const Tensor& pk_, const Tensor& pv_, const 
                   const OptTensor& v_words, bool want_lse) {
   const auto dim = q_.dim();
   if ((dim != 4 && dim != 5) || !q_.is_cuda() || checks_wanted() || k_words.has_value() != v_words.has_value() || wants_grad({&q_, &pk_, &pv_, &k_, &v_})) return py::none();
+  if (k_words.has_value() && k_.scalar_type() != at::kInt) return py::none();  // (refused there)
   const auto dev = q_.get_device();
   for (const Tensor* t : {&pk_, &pv_, &k_, &v_})
     if (t->dim() != dim || !plain_cuda(*t, dev)) return py::none();

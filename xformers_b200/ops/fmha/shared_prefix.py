@@ -38,7 +38,7 @@ _DECODE_BIASES = (
 _OWN_BIASES = _DECODE_BIASES + (ab.BlockDiagonalMask, ab.BlockDiagonalCausalMask, ab.BlockDiagonalCausalFromBottomRightMask)
 
 
-def _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, scale, out_dtype) -> None:
+def _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, scale, out_dtype, k_words, v_words) -> None:
     name = "shared_prefix_attention"
     if query.ndim not in (4, 5) or any(t.ndim != query.ndim for t in (prefix_key, prefix_value, key, value)):
         raise ValueError(f"{name}: query, keys and values must all be [1, M, H, K] or all be [1, M, G, H, K]")
@@ -60,6 +60,8 @@ def _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, 
         raise ValueError(f"{name}: key {tuple(key.shape)} and value {tuple(value.shape)} must have the heads of query {tuple(query.shape)}")
     if prefix_key.dtype != query.dtype or prefix_value.dtype != query.dtype:
         raise ValueError(f"{name}: the prefix must have the dtype of query, got {prefix_key.dtype}, {prefix_value.dtype}")
+    if (k_words is None) != (v_words is None) or (k_words is not None and not key.dtype == value.dtype == torch.int32):
+        raise ValueError(f"{name}: k_fp8_scale_shift and v_fp8_scale_shift go together, with int32 words as key and value, got {key.dtype}, {value.dtype}")
     if any(t.device != query.device for t in (prefix_key, prefix_value, key, value)):
         raise ValueError(f"{name}: all tensors must be on one device")
     rows, slots = prefix_key.shape[1], len(prefix_bias.q_seqinfo.seqstart_py) - 1
@@ -140,7 +142,7 @@ def shared_prefix_attention(
     if torch.is_grad_enabled() and (query.requires_grad or prefix_key.requires_grad or prefix_value.requires_grad or key.requires_grad or value.requires_grad):
         raise NotImplementedError("shared_prefix_attention: an input requires grad, and the backward pass is outside this library; call it under torch.no_grad()")
     out_dtype = output_dtype or query.dtype
-    _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, scale, out_dtype)
+    _check(query, prefix_key, prefix_value, prefix_bias, key, value, attn_bias, scale, out_dtype, k_fp8_scale_shift, v_fp8_scale_shift)
     if query.device.type != "cuda":
         raise ValueError(f"shared_prefix_attention needs CUDA tensors, got device={query.device}")
     fp8 = k_fp8_scale_shift is not None or v_fp8_scale_shift is not None
