@@ -440,8 +440,8 @@ typedef struct {
 XFB200_API int xfb200_rope_padded(const xfb200_rope_params* p, void* stream);
 
 /* The same pass with norms of the queries and keys per head in front of the rotation (no counterpart in the reference): every row x
- * of xq and xk becomes x / sqrt(mean(x^2) + eps) * (w + weight_offset), w the weight of its kind ([dim], contiguous; NULL: ones),
- * before it is rotated and written.  Arithmetic in fp32, rounded once.  dim at most 512.  No row outside [0, cache_rows) of the caches is written,
+ * of xq and xk becomes x / sqrt(mean(x^2) + eps) * (w + weight_offset), w the weight of its kind ([dim], contiguous; NULL: ones,
+ * to which weight_offset is added too), before it is rotated and written.  Arithmetic in fp32, rounded once.  dim at most 512.  No row outside [0, cache_rows) of the caches is written,
  * whatever the page table holds. */
 typedef struct {
   xfb200_rope_params rope;

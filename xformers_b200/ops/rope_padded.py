@@ -132,8 +132,9 @@ def norm_rope_padded(
     (token, head) of ``xq`` and ``xk`` becomes ``x / sqrt(mean(x**2) + eps) * (weight + weight_offset)`` before it is rotated and
     written; ``xv`` is copied.  Statistics and products in float32, rounded once.
 
-    ``q_weight``, ``k_weight``: ``[D]`` in bf16, f16 or f32 (both the same), shared by the heads; ``None`` leaves the weight out (ones).
-    ``weight_offset`` is added to the weights (1 for weights that are stored around zero).  Everything else as in :func:`rope_padded`: caches
+    ``q_weight``, ``k_weight``: ``[D]`` in bf16, f16 or f32 (both the same), shared by the heads; ``None`` stands for a weight of ones.
+    ``weight_offset`` is added to the weights (1 for weights that are stored around zero), to the ones of a missing weight as well: with an offset of 1 it
+    gives a factor of 2, and a plain norm of one kind beside a weight of the other is a weight of zeros.  Everything else as in :func:`rope_padded`: caches
     padded or paged, of the inputs' dtype or quantised as they are written, positions, pair layouts, scalings.  D is even and at
     most 512; a quantised cache needs D of 32, 64, 128, 256 or 512.  A key whose row lies outside its slot or the cache is not written.
     """
