@@ -293,6 +293,8 @@ XFB200_API int xfb200_decode_forward_static_scratch(const xfb200_decode_params* 
  * multiple of 8 tokens).  bf16 or f16, head dim 64 or 128, every query of a group sees its whole prefix.
  * The own keys come in one of two ways: `own`, parameters of the decode kernel (any cache it reads; q, out, lse, scratch, dtype, scale and flags are
  * taken from here), which runs as part of the call; or own_out / own_lse, one fp32 partial per row that another operator has left.
+ * Starts and lengths are read on the device; max_q, total_q and kv_padding are bounds that hold for every replay of a captured call (tokens of a group behind the
+ * max_q-th would not see the prefix).
  *
  * q, out [total_q, kv_heads, q_per_kv, D] (strides m, g, h), k, v [rows, kv_heads, D] (strides m, g; 0 = one for all heads). */
 typedef struct {
