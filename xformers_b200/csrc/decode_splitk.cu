@@ -54,8 +54,6 @@ struct DecodeArgs {
   int32_t page_shift;  // log2(page_size), -1 if that is no power of two
   int32_t split_k, chunk_tokens;
   int32_t beside;         // runs beside the kernel ahead in the stream
-  int32_t partials_only;  // the caller merges the chunks, however many there are
-  int32_t direct;      // one chunk per sequence and no merge behind it: the kernel writes the output itself
   int32_t hb;          // kv heads per CTA (1, 2, 4 or 8)
   int32_t rows;        // R = mq * q_per_kv
   int32_t row_blocks;  // ceil(R / (16*MT))
@@ -88,6 +86,10 @@ struct DecodeArgs {
   int32_t bias_dtype;
   float inv_scale;
   int64_t bias_b, bias_kvh, bias_q, bias_m;
+  // (These last: in front of `hb`, they shift what the loops read, and paged decode of 64 sequences over an fp8 cache takes 367 us instead of 359, bf16 604 and 603,
+  // int4 259.1 and 260.2.)
+  int32_t partials_only;  // the caller merges the chunks, however many there are
+  int32_t direct;         // one chunk per sequence and no merge behind it: the kernel writes the output itself
 };
 
 template <bool kBf16>
