@@ -14,7 +14,7 @@
 //   Three kernels: norm_rope_few_kernel for what fits the SMs at a token to a CTA, norm_rope_kernel for more, norm_rope_any_kernel for rows that do not start on
 // 16-byte boundaries.  Frequencies (a double-precision exponential each) are formed once per CTA, before it waits for the kernel ahead of it in the stream.
 // Measured (bf16, 64 + 2 x 8 rows of 128 a token): 26939 tokens of 9 sequences 185 us (6.0 TB/s; the memory, half of whose traffic are writes, is what bounds it), 8096
-// of 2 sequences 63 (5.2), 2048 of 2048 sequences 18.6 (4.5), 256 of 256 sequences 5.1 (latency).
+// of 2 sequences 62 (5.3), 2048 of 2048 sequences 18.8 (4.5), 256 of 256 sequences 5.2 (latency).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -117,7 +117,7 @@ struct NormShared {
   }
   // Sines and cosines of a token, by its warp.  The angle is formed in double precision and reduced there, to [-pi, pi]: single-precision sine and cosine are only
   // good on a small range.  Their fast forms are off by 2^-21, which 16-bit outputs do not show; fp32 ones get sincospif (417 tokens of 48 rows of 80: error
-  // 1.8e-7 -> 7.8e-8 of the outputs' norm, 6.9 -> 7.3 us).  internal_f64 takes them in double precision.
+  // 1.8e-7 -> 7.8e-8 of the outputs' norm, 7.5 -> 7.6 us).  internal_f64 takes them in double precision.
   __device__ __forceinline__ void angles(const NormRopeArgs& a, double pos, int lane) {
     __syncwarp();
     for (int j = lane; j < a.p.dim / 2; j += 32) {
@@ -326,10 +326,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rope_few_kernel(const __
 
 // ---------------------------------------------------------------------------
 // Many tokens: CTAs that are resident all the time, whose warps go through the tokens of the call as one row of them, whatever the lengths of its sequences.
-// (With CTAs that have up to 16 tokens of one sequence each: 8096 tokens of 2 sequences 81 us instead of 63, a prompt of 2048 beside 63 single tokens, 32 heads, 33.5 instead of 12.8.)
+// (With CTAs that have up to 16 tokens of one sequence each: 8096 tokens of 2 sequences 81 us instead of 62, a prompt of 2048 beside 63 single tokens, 32 heads, 33.5 instead of 12.8.)
 // ---------------------------------------------------------------------------
 // How many warps of a CTA share a token, so that the slowest is through soonest: a token costs a warp as much as kTokenRows steps of rows
-// before the first one.  (1 / 2 / 4 / 8 warps: 8096 tokens of 80 rows of 128 72 / 69 / 73 / 97 us, 540 of them 17.2 / 12.5 / 10.1 / 11.5, by an earlier form of this kernel.)
+// before the first one.  (1 / 2 / 4 / 8 warps, and as this has it: 8096 tokens of 80 rows of 128 62.9 / 61.0 / 68.0 / 88.4, 61.6 us; 1024 of them 13.2 / 10.9 / 12.8 / 16.0, 11.5;
+// 540 12.9 / 8.9 / 8.1 / 9.8, 8.7; 2048 tokens of 48 rows 11.6 / 13.4 / 16.0 / 21.0, 12.2.)
 constexpr int kTokenRows = 3;
 __device__ __forceinline__ int warps_per_token(int64_t tokens, int steps) {
   int best = kNormWarps;
@@ -372,14 +373,15 @@ struct WarpTokens {
   }
 };
 
-// CTAs to an SM: what the registers of 16-bit rows, twice as many elements to a lane, allow (three with spilt registers: 26939 tokens 196 us instead of 187; f32,
-// 17981 tokens of 24 rows of 80: two 71 us, three 64).
+// CTAs to an SM: what the registers of 16-bit rows, twice as many elements to a lane, allow (three with spilt registers: 26939 tokens 198 us instead of 185; f32,
+// 17981 tokens of 24 rows of 80: two 70 us, three 63).
 template <typename T>
 constexpr int norm_ctas() { return sizeof(T) == 4 ? 3 : 2; }
 
 // Rows start on 16-byte boundaries and dim is a multiple of two vectors.  A warp's rows come through a ring in shared memory, kNormDepth - 1 batches ahead and across tokens;
-// every lane copies and reads back its own vectors, so no barrier is involved.  Nothing reads the rows again, so the L2 is told to drop them first (26939 tokens: 204 -> 188 us), and
-// more on the way at once does not help (rings of 3 / 4 batches 186 / 194 us).
+// every lane copies and reads back its own vectors, so no barrier is involved.  Nothing reads the rows again, so the L2 is told to drop them first, which
+// leaves it to what is written (without: 2048 single tokens 19.5 us instead of 18.8, 3563 tokens of 48 rows 21.2 instead of 20.4; 26939 of 80 rows, far beyond the L2, 181
+// instead of 185).  More on the way at once does not help the longest calls (rings of 3 / 4 batches: 26939 tokens 185 / 194 us, 8096 61.6 / 59.4).
 template <typename T, bool kAdj, int kQuant>
 __global__ void __launch_bounds__(kNormThreads, norm_ctas<T>()) norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
   constexpr int E = RopeVec<T>::kElems;

@@ -7,7 +7,7 @@
 // the GQA group) pairs of all sequences of the group, are the M rows of tcgen05 products with tiles of 128 keys.  (2) The split-K decode kernel reads
 // the sequences' own keys and leaves its partials (decode_splitk.cu).  It runs beside (1), which is bound by the tensor cores where it takes
 // long, on the SMs that (1) leaves it.  Or a prefill kernel has left one partial per row, ahead of (1), which then runs beside that one where the caller says that it may (2
-// sequences of 14 tokens and 862 own keys behind 706 keys, 64 heads: 28.6 -> 18.5 us; 8 of up to 300 tokens behind 16384: 407 -> 401).  (3) shared_merge_kernel joins the partials
+// sequences of 14 tokens with 862 and 812 own keys behind 706 keys, 64 heads: 32.0 -> 23.4 us; 4 of 100 tokens behind 3000: 52.5 -> 51.3).  (3) shared_merge_kernel joins the partials
 // of a row in a fixed order.
 //
 // An item of (1) is a block of one or two tiles of 128 rows of one (group, kv head); it takes a step for every 128 keys of the prefix.  The
@@ -973,7 +973,10 @@ static int launch_prefix(const Args& a, dim3 grid, cudaStream_t st) {
 }
 
 // Warps per row: as many as let every warp have its partials in one round of loads, while the rows' warps are resident together; latency is what a
-// few rows cost, getting through CTAs what many do.
+// few rows cost, getting through CTAs what many do.  Measured, us of a call with 1 / 2 / 4 / 8 warps a row, 8 of them with eight loads each (what the rule takes in brackets; 8 kv heads
+// of 128 unless said): one sequence, 8 heads on one kv head, behind 40000 keys 31.8 / 23.8 / 19.5 / 17.7 / [17.0]; 2 of 64 heads behind 65536 60.4 / 57.7 / 56.6 / [56.2] / 56.1; 4 behind 601
+// 12.6 / 12.0 / [11.9] / 12.0 / 12.4; 32 behind 4096 24.9 / 24.0 / [23.7] / 27.2 / 30.1; 48 behind 5000 41.2 / [38.9] / 42.4 / 45.9 / 49.2; 128 of 64 heads behind 8192
+// [149] / 155 / 167 / 186 / 201; 160 tokens of 28 heads in five groups [24.7] / 30.3 / 37.1 / 50.3 / 51.4.
 template <int D>
 static int launch_merge(const MergeArgs& a, int partials, cudaStream_t st) {
   const int64_t rows = int64_t(a.total_q) * a.kv_heads * a.q_per_kv, resident = int64_t(sm_count()) * 32;
@@ -1032,9 +1035,9 @@ static int32_t own_flags(const xfb200_decode_params& own) {
 // of one tile no less than its bytes at its share of the memory's rate; a decode CTA 4 us (two tiles of rows: 8) and its keys at 55 GB/s or its share,
 // of the bounds' three quarters (lengths are not known here).  Decode CTAs that find no free SM start when the first are through; where they come
 // in several waves, which share the memory with the prefix kernel, that one has to be over in the first half.
-// Measured, us by SMs of the prefix kernel (head dim 128; the rule's choice last): 32 sequences behind 4096 keys 148 / 80 / 40 / 32: 30.8 / 28.2 / 26.3 / 26.5;
-// 48 behind 5000 148 / 64 / 32 / 48: 55.7 / 51.7 / 46.1 / 42.2; 128 of 64 heads behind 8192, paged, 148 / 64 / 48 / 32: 166.7 / 155.4 / 150.1 / 148.1; 16 of 64 heads
-// behind 131072 96 / 148 / 128: 123.8 / 105.4 / 103.7.
+// Measured, us by SMs of the prefix kernel (head dim 128; the rule's choice last): 32 sequences behind 4096 keys 148 / 80 / 40 / 24 / 32: 29.9 / 26.4 / 24.1 / 24.8 / 23.3;
+// 48 behind 5000 148 / 64 / 32 / 24 / 48: 55.2 / 49.8 / 38.8 / 44.7 / 38.9; 128 of 64 heads behind 8192, paged, 148 / 64 / 48 / 24 / 32: 166.8 / 156.2 / 151.0 / 178.8 / 149.3; 16 of 64
+// heads behind 131072 96 / 148 / 128: 119.2 / 105.1 / 102.0.
 static int prefix_ctas(const Layout& l, int head_dim, int groups, const xfb200_decode_params& own_) {
   xfb200_decode_params own = own_;
   own.flags = own_flags(own);
@@ -1170,7 +1173,7 @@ extern "C" int xfb200_shared_prefix_forward(const xfb200_shared_prefix_params* p
     int rc = map(&a.tm_k, p->k, p->k_stride_m, p->k_stride_g, &a.k_heads_step);
     if (rc == XFB200_OK) rc = map(&a.tm_v, p->v, p->v_stride_m, p->v_stride_g, &a.v_heads_step);
     if (rc != XFB200_OK) return rc;
-    // Q by tiled copies where 128 rows are whole tokens (4 sequences of 4 rows a kv head behind 601 keys, with stores by the softmax warps and so: 11.5 / 11.0 us; 1754
+    // Q by tiled copies where 128 rows are whole tokens (4 sequences of 4 rows a kv head behind 601 keys, with stores by the softmax warps and so: 11.5 / 11.0 us; 1753
     // tokens behind 16384: 414 / 411)
     if (p->q_per_kv <= kBM && (p->q_per_kv & (p->q_per_kv - 1)) == 0) {
       const int64_t ext[3] = {p->q_per_kv, p->kv_heads, p->total_q}, st[3] = {p->q_stride_h, p->q_stride_g, p->q_stride_m};

@@ -134,8 +134,8 @@ def shared_prefix_attention(
     ``scale > 0``.  Lengths, starts and page tables are read on the device, so a captured call may be replayed after they changed, as long as no group has more
     tokens than the largest one had at the capture.  A token with neither prefix nor own keys gets zeros and ``-inf``.
 
-    It pays from about eight sequences and 15000 keys on that are not read again (prefix keys times sequences but one); below that, decode attention over page tables that
-    repeat the prefix's pages is sooner done (32 query heads on 8 kv heads of 128, 2 sequences behind 4096 keys: 10.9 us, here 15.5).  Where a prefill kernel runs, the
+    It pays from some 16000 keys on that are not read again (prefix keys times sequences but one); below that, decode attention over page tables that
+    repeat the prefix's pages is sooner done (32 query heads on 8 kv heads of 128, 2 sequences behind 4096 keys: 10.4 us, here 15.5).  Where a prefill kernel runs, the
     call holds two fp32 rows of K elements for every query row while it runs, one of the own keys and one or more of the prefix.
 
     Returns the output, with ``return_lse`` ``(out, lse [1, (G,) H, M])``.  No gradients.
