@@ -1426,7 +1426,7 @@ __global__ void __launch_bounds__(kDecThreads, DecOccupancy<kFmt, MT>::kCtasPerS
     mbar_fence_init();
     if (a.copy_mode == 3) prefetch_tensormap(&a.tm_k), prefetch_tensormap(&a.tm_v);
   }
-  // (In this order: the merge reads the lengths before its own wait, so it must not begin before whatever wrote them has ended.)
+  // (In this order: the merge guesses by the lengths ahead of its own wait, and a guess at what is still being written is seldom right.)
   // Beside the kernel ahead (XFB200_DECODE_BESIDE): everything this one reads was complete when that one began.  The launch's last CTA waits for it at
   // its end, so that whoever waits for this kernel has both; the others would only keep their SMs.  (Which one is the last is worked out there: kept from here on, the
   // answer cost four sequences of 1000 keys 11.46 -> 11.70 us, two of 65536 in four segments 53.1 -> 53.9.)
@@ -1773,8 +1773,9 @@ __global__ void __launch_bounds__(kDecThreads, DecOccupancy<kFmt, MT>::kCtasPerS
 // Merge of the per-chunk partials of each sequence.  Latency bounds it, not bytes: what a row needs is asked for in rounds
 // of loads -- the log-sum-exps of all chunks for the maximum, and for each of the row's kWarpsPerRow warps U of its chunks with their
 // log-sum-exps, which do not wait for the maximum (4 sequences of 1000 keys: 9.4 -> 8.5 us for both kernels).  How many warps a row
-// gets is chosen at the launch.  Lengths are read before the split kernel has ended, which is right only because that kernel lets this
-// one begin behind its own wait: whatever wrote the lengths has ended then.
+// gets is chosen at the launch.  Lengths are read ahead of the wait for the split kernel, as a guess that the loads go by, and once more behind it: what was written
+// ahead of that kernel is visible for certain only then.  (Read behind it alone: four sequences of 1000 keys with the append 11.5 -> 12.0 us; with the guess 11.3,
+// and paged decode of 64 sequences 623 -> 627.)
 // Every chunk goes to a fixed warp and the warps are added up in order,
 // whatever the number of chunks, so the result is deterministic and does not
 // depend on a bound.  Only the chunks that exist for sequence b are read.
@@ -1793,9 +1794,13 @@ __global__ void __launch_bounds__(kMergeWarpsPerCta * 32) decode_merge_kernel(co
   const int row = int(gw % R);
   const int head = int((gw / R) % a.kv_heads);
   const int b = live ? int(gw / (int64_t(R) * a.kv_heads)) : 0;
-  int kv_len = a.seqlen_k != nullptr ? min(max(a.seqlen_k[b], 0), a.kv_padding) : a.kv_padding;
-  if (a.window_size > 0) kv_len = min(kv_len, a.window_span);
-  const int nsplit = live ? min(a.split_k, (kv_len + a.chunk_tokens - 1) / a.chunk_tokens) : 0;
+  const int guess = a.seqlen_k != nullptr ? a.seqlen_k[b] : a.kv_padding;
+  auto chunks = [&](int len) -> int {
+    len = min(max(len, 0), a.kv_padding);
+    if (a.window_size > 0) len = min(len, a.window_span);
+    return live ? min(a.split_k, (len + a.chunk_tokens - 1) / a.chunk_tokens) : 0;
+  };
+  int nsplit = chunks(guess);
   const int64_t prow0 = (int64_t(b) * a.split_k * a.kv_heads + head) * R + row, pstep = int64_t(a.kv_heads) * R;
   grid_dep_wait();
   grid_dep_launch();
@@ -1822,8 +1827,14 @@ __global__ void __launch_bounds__(kMergeWarpsPerCta * 32) decode_merge_kernel(co
     }
   };
   load(part);
+  const int len = a.seqlen_k != nullptr ? __ldcg(a.seqlen_k + b) : a.kv_padding;
   float mx = -INFINITY;
   for (int s = lane; s < nsplit; s += 32) mx = fmax_nan(mx, a.part_lse[prow0 + s * pstep]);  // (NaN in any chunk is NaN in all that follows)
+  if (len != guess) {  // (the same for the whole warp)
+    nsplit = chunks(len), mx = -INFINITY;
+    load(part);
+    for (int s = lane; s < nsplit; s += 32) mx = fmax_nan(mx, a.part_lse[prow0 + s * pstep]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float acc[V];

@@ -84,9 +84,8 @@ inline size_t decode_partials_bytes(const xfb200_decode_params& p) {
 }
 
 // Launch that may begin while the kernel ahead of it in the stream still runs.  Only for kernels whose every CTA calls
-// grid_dep_wait() before it touches memory (a kernel launched behind one of the library's own, which lets it begin after its own wait, may
-// read before that what neither writes: decode_merge_kernel the lengths): what is saved is the launch itself and what the kernel does before that call, 1-2 us
-// of a decoding step's 3-6 us kernels.  In a captured stream it becomes an edge of the same kind.
+// grid_dep_wait() before it touches memory (decode_merge_kernel reads lengths ahead of it, and again behind it): what is saved is the
+// launch itself and what the kernel does before that call, 1-2 us of a decoding step's 3-6 us kernels.  In a captured stream it becomes an edge of the same kind.
 //   A kernel that leaves SMs free for other streams (sm_margin) neither is launched this way nor lets the next one begin: CTAs that
 // only wait would fill those SMs.
 //   in_order: an ordinary launch, for the first of two kernels that run beside one another.  What griddepcontrol.wait makes visible, it makes visible to the grid that waits; a
